@@ -20,9 +20,27 @@ constexpr float LOG2E = 1.4426950408889634f;
 // How far a row's scores may pass its running maximum before the sums are rescaled, as a power of two: the probabilities
 // reach 2^8 then, which costs neither bf16 nor fp32 any precision.
 constexpr float SLACK = 8.f;
-// Scaled scores beyond this are taken as differences before scaling: there the rounding of the scaled maximum is no longer
-// small against 1.
+// Scaled scores beyond this are taken as differences before scaling: there the rounding of a scaled maximum, against whose
+// fixed value scores are taken below it, is no longer small against 1.
 constexpr float HUGE_SCORE = 1048576.f;
+
+// The base of probabilities whose running maximum is m, as a power of two (scale: softmax scale times log2 e). Up to
+// HUGE_SCORE it is the rounded product, which is off by as much as 2^-5 there: sums taken on different bases have to be brought
+// to one by these rounded values and no others, so the product is never merged into a sum. Beyond, it is the exact product.
+OASIS_DEV float base_of(float m, float scale) {
+#pragma clang fp contract(off)
+  return m * scale;
+}
+OASIS_DEV bool is_huge(float base) { return fabsf(base) > HUGE_SCORE; }
+// What brings sums on the base of maximum `from` to that of `to`, as a power of two: the difference of the two bases, each a
+// product yet to take or one taken. `to` is finite or +inf; -inf for a `from` of -inf. (Without branches: with them own_kernel
+// of heads of 128 spills a thousand registers.)
+OASIS_DEV float shift(float from, float to, float scale) {
+#pragma clang fp contract(off)
+  const float a = base_of(from, scale), b = base_of(to, scale);
+  const bool ha = is_huge(a), hb = is_huge(b);
+  return fmaf((ha ? from : 0.f) - (hb ? to : 0.f), scale, (ha ? 0.f : a) - (hb ? 0.f : b));
+}
 
 OASIS_DEV f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
@@ -78,25 +96,25 @@ struct Tile {
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
     mx = max_xor32(mx);
-    float at = m * scale;
-    const float top = mx * scale;
-    if (__any(top > at + SLACK || fabsf(at) > HUGE_SCORE)) {
-      const float to = fmaxf(m, mx), now = to * scale;
-      const float alpha = to == m ? 1.f : __builtin_amdgcn_exp2f(fabsf(now) > HUGE_SCORE ? (m - to) * scale : at - now);
+    float at = base_of(m, scale);
+    const float top = base_of(mx, scale);
+    if (__any(top > at + SLACK || is_huge(at))) {
+      const float to = fmaxf(m, mx);
+      const float alpha = to == m ? 1.f : __builtin_amdgcn_exp2f(shift(m, to, scale));
       m = to;
       l *= alpha;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-      at = m == -INFINITY ? 0.f : now;
-      if (__any(fabsf(at) > HUGE_SCORE)) {
-        const float raw = fabsf(at) > HUGE_SCORE ? m : 0.f;
+      at = m == -INFINITY ? 0.f : base_of(m, scale);
+      if (__any(is_huge(at))) {
+        const float raw = is_huge(at) ? m : 0.f;
 #pragma unroll
         for (int t = 0; t < N; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[t][i] -= raw;
-        at = fabsf(at) > HUGE_SCORE ? 0.f : at;
+        at = is_huge(at) ? 0.f : at;
       }
     }
     return at;

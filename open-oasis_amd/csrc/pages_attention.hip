@@ -114,9 +114,10 @@ OASIS_DEV void by_hand(flash::Tile<D>& w, const PagesArgs& a, const int32_t* tab
         for (int j = 0; j < 8; ++j) dot = fmaf(bf2f(w.q[s][j]), bf2f(k[16 * s + 8 * h + j]), dot);
       dot = sum_xor32(dot);
       if (key >= end) continue;
-      const float to = fmaxf(w.m, dot), raw = to == -INFINITY ? 0.f : to;
-      const float alpha = to == w.m ? 1.f : __builtin_amdgcn_exp2f((w.m - to) * a.scale_log2);
-      const float p = __builtin_amdgcn_exp2f((dot - raw) * a.scale_log2);
+      const float to = fmaxf(w.m, dot), raw = to == -INFINITY ? 0.f : to, base = flash::base_of(raw, a.scale_log2);
+      const float alpha = to == w.m ? 1.f : __builtin_amdgcn_exp2f(flash::shift(w.m, raw, a.scale_log2));
+      // on the base that the joins take it to be on
+      const float p = __builtin_amdgcn_exp2f(flash::is_huge(base) ? (dot - raw) * a.scale_log2 : fmaf(dot, a.scale_log2, -base));
       w.m = to;
       w.l = w.l * alpha + (h ? 0.f : p);  // the halves of a wave add up
 #pragma unroll
@@ -283,7 +284,7 @@ struct Walk {
 #pragma unroll
       for (int i = 0; i < S; ++i) {
         const Sum x = wml[i][lr];
-        const float f = __builtin_amdgcn_exp2f((x.m - (m == -INFINITY ? 0.f : m)) * a.scale_log2);
+        const float f = __builtin_amdgcn_exp2f(flash::shift(x.m, m == -INFINITY ? 0.f : m, a.scale_log2));
         l += f * x.l;
         const f32x4* from = reinterpret_cast<const f32x4*>(smem) + i * REGS / 4 * 64 + lane;
 #pragma unroll
@@ -536,11 +537,11 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[x][i]);
     mx = max_xor32(max_xor16(mx));
-    const float to = fmaxf(m, mx), now = to * a.scale_log2, raw = to == -INFINITY ? 0.f : to;
-    const bool huge = fabsf(raw * a.scale_log2) > flash::HUGE_SCORE;
-    const float alpha = to == m ? 1.f : __builtin_amdgcn_exp2f(huge ? (m - to) * a.scale_log2 : m * a.scale_log2 - now);
+    const float to = fmaxf(m, mx), raw = to == -INFINITY ? 0.f : to, base = flash::base_of(raw, a.scale_log2);
+    const bool huge = flash::is_huge(base);
+    const float alpha = to == m ? 1.f : __builtin_amdgcn_exp2f(flash::shift(m, raw, a.scale_log2));
     m = to;
-    const float off = huge ? raw : 0.f, less = huge ? 0.f : raw * a.scale_log2;
+    const float off = huge ? raw : 0.f, less = huge ? 0.f : base;
     bf16x8 pb;  // rounded for the product, as flash::Tile::probs
     float sum = 0.f;
 #pragma unroll
@@ -612,7 +613,7 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const Sum x = wml[w0 + i][lr];
-      const float f = __builtin_amdgcn_exp2f((x.m - (m == -INFINITY ? 0.f : m)) * a.scale_log2);
+      const float f = __builtin_amdgcn_exp2f(flash::shift(x.m, m == -INFINITY ? 0.f : m, a.scale_log2));
       l += f * x.l;
       const float* from = reinterpret_cast<const float*>(smem + (w0 + i) * STAGE) + lane;
 #pragma unroll
@@ -638,7 +639,7 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
     float top = m;
 #pragma unroll 8
     for (int p = 0; p < a.p_splits; ++p) top = fmaxf(top, ml[p].m);
-    const float raw = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f((m - raw) * a.scale_log2);
+    const float raw = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(flash::shift(m, raw, a.scale_log2));
     bool none = l == 0.f;
     l *= f;
 #pragma unroll
@@ -649,7 +650,7 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
       const Sum x = ml[p];
       const bool some = x.m != -INFINITY || x.l != 0.f;
       none = none && !some;
-      const float e = __builtin_amdgcn_exp2f((x.m - raw) * a.scale_log2);
+      const float e = __builtin_amdgcn_exp2f(flash::shift(x.m, raw, a.scale_log2));
       l += some ? e * x.l : 0.f;
       const float* from = a.o + (slot + p) * D;
 #pragma unroll
@@ -735,7 +736,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagesArgs a) {
   bool used[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    f[j] = __builtin_amdgcn_exp2f((x[j].m - at) * a.scale_log2);
+    f[j] = __builtin_amdgcn_exp2f(flash::shift(x[j].m, at, a.scale_log2));
     used[j] = !(x[j].m == -INFINITY && x[j].l == 0.f);
   }
   const uint64_t mask[2] = {__ballot(used[0]), __ballot(used[1])};
