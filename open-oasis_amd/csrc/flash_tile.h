@@ -21,26 +21,31 @@ constexpr float LOG2E = 1.4426950408889634f;
 // reach 2^8 then, which costs neither bf16 nor fp32 any precision.
 constexpr float SLACK = 8.f;
 // Scaled scores beyond this are taken as differences before scaling: there the rounding of a scaled maximum, against whose
-// fixed value scores are taken below it, is no longer small against 1.
-constexpr float HUGE_SCORE = 1048576.f;
+// fixed value scores are taken below it, is no longer small against 1. (2^20, less what keeps a number and SINK below it too.)
+constexpr float HUGE_SCORE = 1048512.f;
+
+// Probabilities are taken 2^-30 times as large as their sum needs: with SLACK a row's are 2^-22 at most, so the sums of up to
+// 2^22 finite values stay finite, whatever the values are (and of 2^30 values up to 2^120). A probability vanishes below 2^-96 of
+// the row's largest instead of 2^-126.
+constexpr float SINK = 30.f;
 
 // The base of probabilities whose running maximum is m, as a power of two (scale: softmax scale times log2 e). Up to
-// HUGE_SCORE it is the rounded product, which is off by as much as 2^-5 there: sums taken on different bases have to be brought
-// to one by these rounded values and no others, so the product is never merged into a sum. Beyond, it is the exact product.
-OASIS_DEV float base_of(float m, float scale) {
-#pragma clang fp contract(off)
-  return m * scale;
-}
+// HUGE_SCORE it is the rounded sum, which is off by as much as 2^-5 there: sums taken on different bases have to be brought
+// to one by these rounded values and no others. Beyond, it is m * scale + SINK exactly.
+OASIS_DEV float base_of(float m, float scale) { return fmaf(m, scale, SINK); }
 OASIS_DEV bool is_huge(float base) { return fabsf(base) > HUGE_SCORE; }
-// What brings sums on the base of maximum `from` to that of `to`, as a power of two: the difference of the two bases, each a
-// product yet to take or one taken. `to` is finite or +inf; -inf for a `from` of -inf. (Without branches: with them own_kernel
-// of heads of 128 spills a thousand registers.)
-OASIS_DEV float shift(float from, float to, float scale) {
-#pragma clang fp contract(off)
-  const float a = base_of(from, scale), b = base_of(to, scale);
-  const bool ha = is_huge(a), hb = is_huge(b);
-  return fmaf((ha ? from : 0.f) - (hb ? to : 0.f), scale, (ha ? 0.f : a) - (hb ? 0.f : b));
+// A base in two: raw * scale + number, one of them taken as a product yet.
+struct Base {
+  float raw, number;
+};
+OASIS_DEV Base split_base(float m, float scale) {
+  const float b = base_of(m, scale);
+  return is_huge(b) ? Base{m, SINK} : Base{0.f, b};
 }
+// What brings sums on the base `from` to the base `to`, as a power of two. A huge base is near one that is not at HUGE_SCORE
+// only, where SINK is a multiple of the other's last place. (Without branches: with them own_kernel of heads of 128 spills a
+// thousand registers.)
+OASIS_DEV float shift(Base from, Base to, float scale) { return fmaf(from.raw - to.raw, scale, from.number - to.number); }
 
 OASIS_DEV f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
@@ -100,7 +105,7 @@ struct Tile {
     const float top = base_of(mx, scale);
     if (__any(top > at + SLACK || is_huge(at))) {
       const float to = fmaxf(m, mx);
-      const float alpha = to == m ? 1.f : __builtin_amdgcn_exp2f(shift(m, to, scale));
+      const float alpha = to == m ? 1.f : __builtin_amdgcn_exp2f(shift(split_base(m, scale), split_base(to, scale), scale));
       m = to;
       l *= alpha;
 #pragma unroll
@@ -114,7 +119,7 @@ struct Tile {
         for (int t = 0; t < N; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[t][i] -= raw;
-        at = is_huge(at) ? 0.f : at;
+        at = is_huge(at) ? SINK : at;
       }
     }
     return at;

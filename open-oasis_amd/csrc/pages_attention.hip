@@ -29,6 +29,12 @@ typedef oasis_page_cache_t Cache;
 struct Sum {
   float m, l;  // running maximum of the raw scores, sum of the probabilities
 };
+struct WaveSum {
+  float m, l;
+  flash::Base base;  // of the probabilities, split once for all that join it
+};
+// what a sum whose maximum is m is joined on: an empty one, any
+OASIS_DEV flash::Base top_base(float m, float scale) { return flash::split_base(m == -INFINITY ? 0.f : m, scale); }
 
 struct PagesArgs {
   Cache c;
@@ -114,10 +120,10 @@ OASIS_DEV void by_hand(flash::Tile<D>& w, const PagesArgs& a, const int32_t* tab
         for (int j = 0; j < 8; ++j) dot = fmaf(bf2f(w.q[s][j]), bf2f(k[16 * s + 8 * h + j]), dot);
       dot = sum_xor32(dot);
       if (key >= end) continue;
-      const float to = fmaxf(w.m, dot), raw = to == -INFINITY ? 0.f : to, base = flash::base_of(raw, a.scale_log2);
-      const float alpha = to == w.m ? 1.f : __builtin_amdgcn_exp2f(flash::shift(w.m, raw, a.scale_log2));
-      // on the base that the joins take it to be on
-      const float p = __builtin_amdgcn_exp2f(flash::is_huge(base) ? (dot - raw) * a.scale_log2 : fmaf(dot, a.scale_log2, -base));
+      const float to = fmaxf(w.m, dot);
+      const flash::Base base = top_base(to, a.scale_log2);  // as in settle: the joins take it to be this one
+      const float alpha = to == w.m ? 1.f : __builtin_amdgcn_exp2f(flash::shift(flash::split_base(w.m, a.scale_log2), base, a.scale_log2));
+      const float p = __builtin_amdgcn_exp2f(fmaf(dot - base.raw, a.scale_log2, -base.number));
       w.m = to;
       w.l = w.l * alpha + (h ? 0.f : p);  // the halves of a wave add up
 #pragma unroll
@@ -142,7 +148,7 @@ struct Walk {
   static constexpr int SMEM = S * STAGE > MERGE ? S * STAGE : MERGE;
   static_assert(LPW * RPB == 2 * KT && NG * 16 == LPW * RPB && LPW <= 63, "loads");
 
-  static OASIS_WALK void go(const PagesArgs& a, const Part& pt, char* smem, Sum (*wml)[32], int* missing) {
+  static OASIS_WALK void go(const PagesArgs& a, const Part& pt, char* smem, WaveSum (*wml)[32], int* missing) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 31, h = lane >> 5;
     const int hk = (int)a.c.n_kv_heads, ps = (int)a.c.page_size;
@@ -274,17 +280,18 @@ struct Walk {
 #pragma unroll
       for (int r = 0; r < REGS; r += 4)
         mine[r / 4 * 64] = f32x4{w.o[r / 16][r % 16], w.o[r / 16][r % 16 + 1], w.o[r / 16][r % 16 + 2], w.o[r / 16][r % 16 + 3]};
-      if (h == 0) wml[wave][lr] = Sum{w.m, lsum};
+      if (h == 0) wml[wave][lr] = WaveSum{w.m, lsum, flash::split_base(w.m, a.scale_log2)};
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < S; ++i) m = fmaxf(m, wml[i][lr].m);
       l = 0.f;
 #pragma unroll
       for (int r = 0; r < SHARE; ++r) y[r] = 0.f;
+      const flash::Base base = top_base(m, a.scale_log2);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        const Sum x = wml[i][lr];
-        const float f = __builtin_amdgcn_exp2f(flash::shift(x.m, m == -INFINITY ? 0.f : m, a.scale_log2));
+        const WaveSum x = wml[i][lr];
+        const float f = __builtin_amdgcn_exp2f(flash::shift(x.base, base, a.scale_log2));
         l += f * x.l;
         const f32x4* from = reinterpret_cast<const f32x4*>(smem) + i * REGS / 4 * 64 + lane;
 #pragma unroll
@@ -377,7 +384,7 @@ struct Crowd {
 template <int D, int R>
 using Kind = typename std::conditional<R == 8, Crowd<D>, Walk<D>>::type;
 template <int D, int R>
-OASIS_DEV void prefix_part(const PagesArgs& a, int id, char* smem, Sum (*wml)[32], int* missing) {
+OASIS_DEV void prefix_part(const PagesArgs& a, int id, char* smem, WaveSum (*wml)[32], int* missing) {
   const int lane = threadIdx.x & 63, hk = (int)a.c.n_kv_heads;
   Part p;
   constexpr int COLS = 32 * R;
@@ -441,7 +448,7 @@ OASIS_DEV int dim_of(int r, int g) { return r / 4 * 16 + 4 * g + r % 4; }
 // tiles of 32 keys in turn. A wave's keys go to registers, one tile ahead; its values through LDS, where they are transposed
 // on the read.
 template <int D, int S>
-OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32]) {
+OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, WaveSum (*wml)[32]) {
   constexpr int KT = 32, ROW = D * 2, STAGE = KT * ROW, RPB = 1024 / ROW, DS = D / 32, DT = D / 16, REGS = D / 4, SHARE = REGS / S;
   static_assert(REGS * 256 <= STAGE && SHARE * S == REGS, "the sums fit where the values were");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -501,6 +508,7 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
   bf16x8 q[DS];
   f32x4 o[DT];
   float m = -INFINITY, l = 0.f;
+  flash::Base was{-INFINITY, 0.f};
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   f32x4 s[2];
@@ -537,18 +545,18 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[x][i]);
     mx = max_xor32(max_xor16(mx));
-    const float to = fmaxf(m, mx), raw = to == -INFINITY ? 0.f : to, base = flash::base_of(raw, a.scale_log2);
-    const bool huge = flash::is_huge(base);
-    const float alpha = to == m ? 1.f : __builtin_amdgcn_exp2f(flash::shift(m, raw, a.scale_log2));
+    const float to = fmaxf(m, mx);
+    const flash::Base base = top_base(to, a.scale_log2);
+    const float alpha = __builtin_amdgcn_exp2f(flash::shift(was, base, a.scale_log2));
+    was = base;
     m = to;
-    const float off = huge ? raw : 0.f, less = huge ? 0.f : base;
     bf16x8 pb;  // rounded for the product, as flash::Tile::probs
     float sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[x][i] - off, a.scale_log2, -less));
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[x][i] - base.raw, a.scale_log2, -base.number));
         sum += p;
         pb[4 * x + i] = f2bf(p);
       }
@@ -602,7 +610,7 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
     float* mine = reinterpret_cast<float*>(smem + wave * STAGE) + lane;
 #pragma unroll
     for (int r = 0; r < REGS; ++r) mine[r * 64] = o[r / 4][r % 4];
-    if (g == 0) wml[wave][lr] = Sum{m, l};
+    if (g == 0) wml[wave][lr] = WaveSum{m, l, flash::split_base(m, a.scale_log2)};
     __syncthreads();
     const int w0 = wave - sg;
 #pragma unroll
@@ -610,10 +618,11 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
     l = 0.f;
 #pragma unroll
     for (int r = 0; r < SHARE; ++r) y[r] = 0.f;
+    const flash::Base base = top_base(m, a.scale_log2);
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const Sum x = wml[w0 + i][lr];
-      const float f = __builtin_amdgcn_exp2f(flash::shift(x.m, m == -INFINITY ? 0.f : m, a.scale_log2));
+      const WaveSum x = wml[w0 + i][lr];
+      const float f = __builtin_amdgcn_exp2f(flash::shift(x.base, base, a.scale_log2));
       l += f * x.l;
       const float* from = reinterpret_cast<const float*>(smem + (w0 + i) * STAGE) + lane;
 #pragma unroll
@@ -639,7 +648,8 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
     float top = m;
 #pragma unroll 8
     for (int p = 0; p < a.p_splits; ++p) top = fmaxf(top, ml[p].m);
-    const float raw = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(flash::shift(m, raw, a.scale_log2));
+    const flash::Base base = top_base(top, a.scale_log2);
+    const float f = __builtin_amdgcn_exp2f(flash::shift(flash::split_base(m, a.scale_log2), base, a.scale_log2));
     bool none = l == 0.f;
     l *= f;
 #pragma unroll
@@ -650,7 +660,7 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, Sum (*wml)[32
       const Sum x = ml[p];
       const bool some = x.m != -INFINITY || x.l != 0.f;
       none = none && !some;
-      const float e = __builtin_amdgcn_exp2f(flash::shift(x.m, raw, a.scale_log2));
+      const float e = __builtin_amdgcn_exp2f(flash::shift(flash::split_base(x.m, a.scale_log2), base, a.scale_log2));
       l += some ? e * x.l : 0.f;
       const float* from = a.o + (slot + p) * D;
 #pragma unroll
@@ -681,14 +691,14 @@ constexpr int OWN_SMEM(int D) { return NW * 64 * D; }  // NW * STAGE of own_part
 template <int D, int S>
 __global__ __launch_bounds__(NW * 64, 4) void own_kernel(PagesArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[OWN_SMEM(D)];
-  __shared__ Sum wml[NW][32];
+  __shared__ WaveSum wml[NW][32];
   own_part<D, S>(a, blockIdx.x, smem, wml);
 }
 
 template <int D, int R>
 __global__ __launch_bounds__(NW * 64, D == 64 && R < 8 ? 4 : 2) void prefix_kernel(PagesArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[Kind<D, R>::SMEM];
-  __shared__ Sum wml[NW][32];
+  __shared__ WaveSum wml[NW][32];
   __shared__ int missing;
   if (threadIdx.x == 0) missing = 0;
   __syncthreads();
@@ -700,7 +710,7 @@ template <int D, int R>
 __global__ __launch_bounds__(NW * 64, D == 64 && R < 8 ? 4 : 2) void both_kernel(PagesArgs a, int prefixes) {
   constexpr int SMEM = Kind<D, R>::SMEM > OWN_SMEM(D) ? Kind<D, R>::SMEM : OWN_SMEM(D);
   __shared__ __attribute__((aligned(1024))) char smem[SMEM];
-  __shared__ Sum wml[NW][32];
+  __shared__ WaveSum wml[NW][32];
   __shared__ int missing;
   if ((int)blockIdx.x < prefixes) {
     if (threadIdx.x == 0) missing = 0;
@@ -731,12 +741,13 @@ __global__ __launch_bounds__(256) void join_kernel(PagesArgs a) {
 #pragma unroll
   for (int j = 0; j < 2; ++j)
     if (lane + 64 * j < p0) x[j] = Sum{-INFINITY, 0.f};
-  const float m = wave_max(fmaxf(x[0].m, x[1].m)), at = m == -INFINITY ? 0.f : m;
+  const float m = wave_max(fmaxf(x[0].m, x[1].m));
+  const flash::Base base = top_base(m, a.scale_log2);
   float y[V] = {}, f[2];
   bool used[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    f[j] = __builtin_amdgcn_exp2f(flash::shift(x[j].m, at, a.scale_log2));
+    f[j] = __builtin_amdgcn_exp2f(flash::shift(flash::split_base(x[j].m, a.scale_log2), base, a.scale_log2));
     used[j] = !(x[j].m == -INFINITY && x[j].l == 0.f);
   }
   const uint64_t mask[2] = {__ballot(used[0]), __ballot(used[1])};
