@@ -41,6 +41,8 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle 
 
 def launch(device, name, *args):
     """L.call on the current stream of a device (its number), which is made the current device where it is not."""
+    if device < 0:
+        raise L.OasisError(name, -5, "expected device tensors, got some in host memory")
     if torch.cuda.current_device() != device:
         with torch.cuda.device(device):
             L.call(name, *args, _raw_stream(device))
