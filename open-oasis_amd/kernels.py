@@ -65,6 +65,11 @@ def check_heads(what, t, rows, heads, head_dim, device):
         raise L.OasisError(what, -5, "a row's heads must be contiguous, got strides %s" % (t.stride(),))
 
 
+def pitch(t):
+    """Elements from one row of t [rows, heads, head_dim] to the next; of a single row, whose stride may be anything, its own."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
 def check_ints(what, device, *ts):
     """ts are contiguous int32 vectors on the device (its number)."""
     for t in ts:
@@ -213,8 +218,8 @@ def make_prompt_attention_kernel(n_heads, n_kv_heads, head_dim, scale_val):
         n = cu_seqlens.numel() - 1
         if n < 0:
             raise L.OasisError("prompt_attention", -2, "cu_seqlens is empty")
-        launch(dev, "oasis_prompt_attention", q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-               out.data_ptr(), out.stride(0), cu_seqlens.data_ptr(), n, rows, n_heads, n_kv_heads, head_dim, scale_val)
+        launch(dev, "oasis_prompt_attention", q.data_ptr(), pitch(q), k.data_ptr(), pitch(k), v.data_ptr(), pitch(v),
+               out.data_ptr(), pitch(out), cu_seqlens.data_ptr(), n, rows, n_heads, n_kv_heads, head_dim, scale_val)
     return prompt_attention_kernel
 
 

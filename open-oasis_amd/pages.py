@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib as L
-from .kernels import check_heads, check_ints, launch
+from .kernels import check_heads, check_ints, launch, pitch
 
 REFUSALS = {L.PAGES_FULL: "too few free pages",
             L.PAGES_BAD_CALL: "a reserve or fork named a sequence that is not there, twice, or not empty, or too many tokens",
@@ -64,7 +64,7 @@ class PageCache:
         rows = k.shape[0]
         check_heads("write", k, rows, self.n_kv_heads, self.head_dim, self._dev)
         check_heads("write", v, rows, self.n_kv_heads, self.head_dim, self._dev)
-        launch(self._dev, "oasis_pages_write", self._ref, layer, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+        launch(self._dev, "oasis_pages_write", self._ref, layer, k.data_ptr(), pitch(k), v.data_ptr(), pitch(v),
                seqs.data_ptr(), cu.data_ptr(), seqs.numel(), rows)
 
     def fork(self, parents, children, copy=False):
@@ -124,7 +124,7 @@ def make_prefix_attention_kernel(cache, n_heads, scale_val, max_rows, max_groups
         if seqs.numel() != rows or rows > max_rows or groups > max_groups:
             raise L.OasisError("prefix_attention", -2, "%d rows of %d sequences in %d groups; the kernel was made for %d and %d"
                                % (rows, seqs.numel(), groups, max_rows, max_groups))
-        launch(dev, "oasis_pages_attention", cache._ref, layer, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0),
+        launch(dev, "oasis_pages_attention", cache._ref, layer, q.data_ptr(), pitch(q), out.data_ptr(), pitch(out),
                seqs.data_ptr(), rows, cu_groups.data_ptr() if groups else None, prefix_lens.data_ptr() if groups else None,
                groups, max_len, n_heads, scale_val, at, workspace.numel())
     return prefix_attention_kernel

@@ -1,0 +1,39 @@
+"""Calls that the documentation of prompts, cache pages and attention over them allows, beside those of every day."""
+import pytest
+import torch
+
+from helpers import L, pkg
+from test_gpu_pages import Model, branches, check_attention, cumulated, extend, filled, ints, new_cache, reference
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+def near(out, ref, mass):
+    # bf16 rounds to within 2^-8: each probability (the sum divided by is of the unrounded ones) and the output; 1.02
+    # covers the fp32 scores and sums
+    return ((out.double() - ref).abs() <= 1.02 * 2.0 ** -8 * (mass + ref.abs())).all()
+
+
+@pytest.mark.parametrize("pitch", [64, 0, 1, 1 << 25])
+def test_the_stride_of_a_single_row_is_anything(pitch):
+    """torch gives a dim of one any stride: a transposed view's is that of another dim."""
+    hq, hk, d = 4, 2, 64
+    x = torch.randn(8, d, device="cuda").to(BF)
+    q, k, v = (x[a:b].as_strided((1, b - a, d), (pitch, d, 1), x[a:b].storage_offset()) for a, b in ((0, 4), (4, 6), (6, 8)))
+    flat = torch.zeros(hq, d, dtype=BF, device="cuda")
+    out = flat.as_strided((1, hq, d), (pitch, d, 1))
+    pkg.kernels.make_prompt_attention_kernel(hq, hk, d, 0.125)(q, k, v, ints([0, 1]), out)
+    assert torch.equal(flat, x[6:8].repeat_interleave(2, 0))
+    c = pkg.PageCache(1, 4, 16, hk, d, 2, 2)
+    c.reserve(ints([1]), ints([0, 1]))
+    c.write(0, k, v, ints([1]), ints([0, 1]))
+    flat.zero_()
+    pkg.make_prefix_attention_kernel(c, hq, 0.125, 1, 0, 16)(0, q, ints([1]), None, None, out)
+    c.check()
+    assert torch.equal(flat, x[6:8].repeat_interleave(2, 0))
+    turned = x[:4].unsqueeze(1).transpose(0, 1)    # [1, 4, 64], as a projection's heads come
+    assert turned.stride(0) == 64
+    pkg.make_prefix_attention_kernel(c, hq, 0.125, 1, 0, 16)(0, turned, ints([1]), None, None, out)
+    assert torch.equal(flat, x[6:8].repeat_interleave(2, 0))
