@@ -51,23 +51,20 @@ def launch(device, name, *args):
 
 
 def check_heads(what, t, rows, heads, head_dim, device):
-    """t is a bf16 tensor [rows, heads, head_dim] on the device (its number), each row's heads contiguous."""
-    if (t.dtype is torch.bfloat16 and t.shape == (rows, heads, head_dim) and t.get_device() == device >= 0
-            and t.stride()[1:] == (head_dim, 1)):
-        return
-    if t.dtype != torch.bfloat16:
-        raise L.OasisError(what, -3, "expected bf16 tensors, got %s" % t.dtype)
-    if t.shape != (rows, heads, head_dim):
-        raise L.OasisError(what, -2, "expected a tensor [%d, %d, %d], got %s" % (rows, heads, head_dim, tuple(t.shape)))
-    if t.get_device() != device or device < 0:
-        raise L.OasisError(what, -5, "expected device tensors, all on one device, got one on %s" % t.device)
-    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim):
-        raise L.OasisError(what, -5, "a row's heads must be contiguous, got strides %s" % (t.stride(),))
-
-
-def pitch(t):
-    """Elements from one row of t [rows, heads, head_dim] to the next; of a single row, whose stride may be anything, its own."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    """t is a bf16 tensor [rows, heads, head_dim] on the device (its number), each row's heads contiguous. Returns the
+    elements from one row to the next; of a single row, whose stride may be anything, its own."""
+    strides = t.stride()
+    if not (t.dtype is torch.bfloat16 and t.shape == (rows, heads, head_dim) and t.get_device() == device >= 0
+            and strides[1:] == (head_dim, 1)):
+        if t.dtype != torch.bfloat16:
+            raise L.OasisError(what, -3, "expected bf16 tensors, got %s" % t.dtype)
+        if t.shape != (rows, heads, head_dim):
+            raise L.OasisError(what, -2, "expected a tensor [%d, %d, %d], got %s" % (rows, heads, head_dim, tuple(t.shape)))
+        if t.get_device() != device or device < 0:
+            raise L.OasisError(what, -5, "expected device tensors, all on one device, got one on %s" % t.device)
+        if strides[2] != 1 or (heads > 1 and strides[1] != head_dim):
+            raise L.OasisError(what, -5, "a row's heads must be contiguous, got strides %s" % (strides,))
+    return strides[0] if rows > 1 else heads * head_dim
 
 
 def check_ints(what, device, *ts):
@@ -210,16 +207,16 @@ def make_prompt_attention_kernel(n_heads, n_kv_heads, head_dim, scale_val):
     they are. head_dim is 64 or 128."""
     def prompt_attention_kernel(q, k, v, cu_seqlens, out):
         rows, dev = q.shape[0], q.get_device()
-        check_heads("prompt_attention", q, rows, n_heads, head_dim, dev)
-        check_heads("prompt_attention", k, rows, n_kv_heads, head_dim, dev)
-        check_heads("prompt_attention", v, rows, n_kv_heads, head_dim, dev)
-        check_heads("prompt_attention", out, rows, n_heads, head_dim, dev)
+        ld_q = check_heads("prompt_attention", q, rows, n_heads, head_dim, dev)
+        ld_k = check_heads("prompt_attention", k, rows, n_kv_heads, head_dim, dev)
+        ld_v = check_heads("prompt_attention", v, rows, n_kv_heads, head_dim, dev)
+        ld_out = check_heads("prompt_attention", out, rows, n_heads, head_dim, dev)
         check_ints("prompt_attention", dev, cu_seqlens)
         n = cu_seqlens.numel() - 1
         if n < 0:
             raise L.OasisError("prompt_attention", -2, "cu_seqlens is empty")
-        launch(dev, "oasis_prompt_attention", q.data_ptr(), pitch(q), k.data_ptr(), pitch(k), v.data_ptr(), pitch(v),
-               out.data_ptr(), pitch(out), cu_seqlens.data_ptr(), n, rows, n_heads, n_kv_heads, head_dim, scale_val)
+        launch(dev, "oasis_prompt_attention", q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, out.data_ptr(), ld_out,
+               cu_seqlens.data_ptr(), n, rows, n_heads, n_kv_heads, head_dim, scale_val)
     return prompt_attention_kernel
 
 

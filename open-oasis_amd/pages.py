@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib as L
-from .kernels import check_heads, check_ints, launch, pitch
+from .kernels import check_heads, check_ints, launch
 
 REFUSALS = {L.PAGES_FULL: "too few free pages",
             L.PAGES_BAD_CALL: "a reserve or fork named a sequence that is not there, twice, or not empty, or too many tokens",
@@ -62,9 +62,9 @@ class PageCache:
         """The keys and values [rows, n_kv_heads, head_dim] of the tokens reserved last with the same seqs and cu."""
         self._lists("write", seqs, cu)
         rows = k.shape[0]
-        check_heads("write", k, rows, self.n_kv_heads, self.head_dim, self._dev)
-        check_heads("write", v, rows, self.n_kv_heads, self.head_dim, self._dev)
-        launch(self._dev, "oasis_pages_write", self._ref, layer, k.data_ptr(), pitch(k), v.data_ptr(), pitch(v),
+        ld_k = check_heads("write", k, rows, self.n_kv_heads, self.head_dim, self._dev)
+        ld_v = check_heads("write", v, rows, self.n_kv_heads, self.head_dim, self._dev)
+        launch(self._dev, "oasis_pages_write", self._ref, layer, k.data_ptr(), ld_k, v.data_ptr(), ld_v,
                seqs.data_ptr(), cu.data_ptr(), seqs.numel(), rows)
 
     def fork(self, parents, children, copy=False):
@@ -112,8 +112,8 @@ def make_prefix_attention_kernel(cache, n_heads, scale_val, max_rows, max_groups
 
     def prefix_attention_kernel(layer, q, seqs, cu_groups, prefix_lens, out):
         rows = q.shape[0]
-        check_heads("prefix_attention", q, rows, n_heads, dim, dev)
-        check_heads("prefix_attention", out, rows, n_heads, dim, dev)
+        ld_q = check_heads("prefix_attention", q, rows, n_heads, dim, dev)
+        ld_out = check_heads("prefix_attention", out, rows, n_heads, dim, dev)
         check_ints("prefix_attention", dev, seqs)
         groups = 0
         if cu_groups is not None:
@@ -124,7 +124,7 @@ def make_prefix_attention_kernel(cache, n_heads, scale_val, max_rows, max_groups
         if seqs.numel() != rows or rows > max_rows or groups > max_groups:
             raise L.OasisError("prefix_attention", -2, "%d rows of %d sequences in %d groups; the kernel was made for %d and %d"
                                % (rows, seqs.numel(), groups, max_rows, max_groups))
-        launch(dev, "oasis_pages_attention", cache._ref, layer, q.data_ptr(), pitch(q), out.data_ptr(), pitch(out),
+        launch(dev, "oasis_pages_attention", cache._ref, layer, q.data_ptr(), ld_q, out.data_ptr(), ld_out,
                seqs.data_ptr(), rows, cu_groups.data_ptr() if groups else None, prefix_lens.data_ptr() if groups else None,
                groups, max_len, n_heads, scale_val, at, workspace.numel())
     return prefix_attention_kernel
