@@ -111,6 +111,8 @@ def make_prefix_attention_kernel(cache, n_heads, scale_val, max_rows, max_groups
     dev, dim, at = cache._dev, cache.head_dim, workspace.data_ptr()
 
     def prefix_attention_kernel(layer, q, seqs, cu_groups, prefix_lens, out):
+        if (cu_groups is None) != (prefix_lens is None):
+            raise L.OasisError("prefix_attention", -1, "cu_groups and prefix_lens come together, or neither")
         rows = q.shape[0]
         ld_q = check_heads("prefix_attention", q, rows, n_heads, dim, dev)
         ld_out = check_heads("prefix_attention", out, rows, n_heads, dim, dev)
