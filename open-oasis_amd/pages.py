@@ -31,6 +31,9 @@ class PageCache:
 
     def __init__(self, n_layers, n_pages, page_size, n_kv_heads, head_dim, max_seqs, max_pages, device="cuda"):
         dev = torch.device(device)
+        sizes = n_layers, n_pages, page_size, n_kv_heads, head_dim, max_seqs, max_pages
+        # a call of no sequences looks at the sizes and at no memory
+        L.call("oasis_pages_truncate", ctypes.byref(L.PageCache(*[16] * 7, *sizes)), None, None, 0, None)
         work = L.count("oasis_pages_work", n_pages, max_seqs)
         shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
         self.n_layers, self.page_size, self.n_kv_heads, self.head_dim = n_layers, page_size, n_kv_heads, head_dim
@@ -43,7 +46,7 @@ class PageCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._work = torch.empty(work, dtype=torch.int32, device=dev)
         p = [t.data_ptr() for t in (self.k, self.v, self.refs, self.tables, self.lens, self.status, self._work)]
-        self.struct = L.PageCache(*p, n_layers, n_pages, page_size, n_kv_heads, head_dim, max_seqs, max_pages)
+        self.struct = L.PageCache(*p, *sizes)
         self._ref = ctypes.byref(self.struct)
         self._dev = self.refs.get_device()
 

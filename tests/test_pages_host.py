@@ -23,3 +23,12 @@ def test_group_bounds_and_prefix_lengths_come_together():
     for bounds, prefix in ((two, None), (None, two[:1])):
         with pytest.raises(L.OasisError, match="together"):
             f(0, q, two, bounds, prefix, q)
+
+
+@pytest.mark.parametrize("change,needle", [
+    (dict(page_size=24), "page_size"), (dict(page_size=2048), "page_size"), (dict(head_dim=96), "head_dim"), (dict(max_seqs=65537), "shape"),
+    (dict(n_layers=0), "shape"), (dict(n_kv_heads=-1), "shape"), (dict(max_pages=0), "shape"), (dict(max_seqs=-3), "shape"), (dict(n_pages=0), "shape")])
+def test_a_cache_of_sizes_that_no_call_takes_is_refused_before_its_pools_are_allocated(change, needle):
+    sizes = dict(n_layers=60000, n_pages=1 << 27, page_size=16, n_kv_heads=1000, head_dim=64, max_seqs=4, max_pages=8)
+    with pytest.raises(L.OasisError, match=needle):
+        pkg.PageCache(**(sizes | change), device="cpu")     # pools past all memory
