@@ -1,10 +1,15 @@
 """What the Python surface of prompts and cache pages refuses or takes on the host, before any device work."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
 from helpers import L, pkg
 
 BF = torch.bfloat16
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_no_call_launches_on_a_cache_in_host_memory():
@@ -32,3 +37,18 @@ def test_a_cache_of_sizes_that_no_call_takes_is_refused_before_its_pools_are_all
     sizes = dict(n_layers=60000, n_pages=1 << 27, page_size=16, n_kv_heads=1000, head_dim=64, max_seqs=4, max_pages=8)
     with pytest.raises(L.OasisError, match=needle):
         pkg.PageCache(**(sizes | change), device="cpu")     # pools past all memory
+
+
+def test_the_package_imports_where_torch_has_no_device_backend():
+    """As before the serving calls: their way to the current stream is looked for when the first of them launches."""
+    code = """
+import torch
+for name in [n for n in vars(torch._C) if n.startswith("_cuda_")]:
+    delattr(torch._C, name)
+from __graft_entry__ import load_package
+pkg = load_package()
+assert pkg.PageCache(1, 4, 16, 2, 64, 2, 2, device="cpu").page_size == 16
+print("imported")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "imported" in r.stdout, r.stderr[-2000:]
