@@ -781,8 +781,8 @@ enum {
   OASIS_PAGES_BAD_CALL = 2, /* a reserve or fork named a sequence that is not there, or twice, a child
                                that is not empty or is also a parent, or tokens that are negative in
                                number or past max_pages: it changed nothing                          */
-  OASIS_PAGES_BAD_ENTRY = 4 /* a truncate or write skipped an entry: a sequence, length or page that is
-                               not there                                                             */
+  OASIS_PAGES_BAD_ENTRY = 4 /* a truncate or write skipped an entry: a sequence, length, page or row that
+                               is not there                                                          */
 };
 /* While FULL or BAD_CALL is set, reserve, write, fork and compact do nothing (truncate works, so pages can be freed):
  * what follows a refused call in a stream or graph does not run on lengths that it never got. */
@@ -798,7 +798,8 @@ int oasis_pages_reserve(const oasis_page_cache_t* cache, const int32_t* seqs, co
 
 /* The keys and values of the last cu[i+1] - cu[i] tokens of each sequence seqs[i], in one layer: rows cu[i] .. of k and v
  * [total, n_kv_heads, head_dim], ld_* elements apart (multiples of 8). Follows the reserve with the same seqs and cu.
- * Rows outside [cu[0], cu[n]) are not read. */
+ * Rows outside [cu[0], cu[n]) are not read. Tokens without a row (cu[0] < 0, cu[n] > total) are skipped, which sets
+ * BAD_ENTRY; a call with total = 0 does nothing at all. */
 int oasis_pages_write(const oasis_page_cache_t* cache, int64_t layer, const void* k, int64_t ld_k, const void* v,
                       int64_t ld_v, const int32_t* seqs, const int32_t* cu, int64_t n, int64_t total,
                       oasis_stream_t stream);

@@ -427,6 +427,7 @@ __global__ __launch_bounds__(256) void write_kernel(Cache c, int64_t layer, cons
     if (in(tid + j * 256)) load(tid + j * 256, &a[j], &b[j]);
   __syncthreads();
   if (refused) return;
+  if (blockIdx.x == 0 && tid == 0 && (lo < 0 || hi > total)) atomicOr(c.status, OASIS_PAGES_BAD_ENTRY);  // tokens without rows
   const int32_t* cus = n < FEW ? near : cu;
   if (tid < rows) {
     const int64_t t = t0 + tid;

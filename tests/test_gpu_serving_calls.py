@@ -37,3 +37,28 @@ def test_the_stride_of_a_single_row_is_anything(pitch):
     assert turned.stride(0) == 64
     pkg.make_prefix_attention_kernel(c, hq, 0.125, 1, 0, 16)(0, turned, ints([1]), None, None, out)
     assert torch.equal(flat, x[6:8].repeat_interleave(2, 0))
+
+
+@pytest.mark.parametrize("bounds,rows", [([0, 3, 8], 7), ([0, 3, 8], 1), ([-2, 3, 8], 8)])
+def test_a_write_of_fewer_rows_than_its_tokens_is_reported(bounds, rows):
+    """Those that are there are written, the others' slots stay as they were, and check() says so."""
+    c = new_cache()
+    m = Model(c)
+    counts = [bounds[1] - bounds[0], 5]
+    c.reserve(ints([2, 0]), cumulated(counts))
+    m.reserve([2, 0], counts)
+    c.check()
+    k = torch.randn(rows, 2, 64, device="cuda").to(BF)
+    c.write(1, k, -k, ints([2, 0]), ints(bounds))
+    assert int(c.status) == L.PAGES_BAD_ENTRY
+    for s, at in ((2, bounds[0]), (0, 3)):
+        for pos in range(m.lens[s]):
+            if 0 <= at + pos < rows:
+                p, slot = m.tables[s][pos // 16], pos % 16
+                m.k[1, p, :, slot], m.v[1, p, :, slot] = k[at + pos].cpu(), -k[at + pos].cpu()
+    m.check(c)
+    with pytest.raises(L.OasisError, match="row"):
+        c.check()
+    spare = torch.randn(20, 2, 64, device="cuda").to(BF)     # more rows than tokens are none of its business
+    c.write(1, spare, -spare, ints([2, 0]), cumulated(counts))
+    c.check()
