@@ -782,7 +782,8 @@ enum {
                                that is not empty or is also a parent, or tokens that are negative in
                                number or past max_pages: it changed nothing                          */
   OASIS_PAGES_BAD_ENTRY = 4 /* a truncate or write skipped an entry: a sequence, length, page or row that
-                               is not there                                                          */
+                               is not there; or a fork gave a child its parent's table entry that names
+                               no page                                                               */
 };
 /* While FULL or BAD_CALL is set, reserve, write, fork and compact do nothing (truncate works, so pages can be freed):
  * what follows a refused call in a stream or graph does not run on lengths that it never got. */

@@ -3,9 +3,10 @@
 // Every sequence's tokens lie in pages of page_size tokens, which its row of `tables` names in order; `refs` counts the
 // sequences on each page, and a page with none is free. Free pages are handed out lowest number first, in the order of the
 // call's sequences, so the same calls give the same tables. Reserving, forking and compacting are planned by one workgroup
-// (prefix sums over the sequences, then over the pages' references), which checks the whole call before it changes
-// anything; what it plans (page copies, table entries) is carried out by launches over the whole chip. Cutting sequences
-// and writing tokens need no plan.
+// (prefix sums over the sequences, then over the pages' references), which checks the call's sequences, lengths and need of
+// pages before it changes anything; what it plans (page copies, table entries) is carried out by launches over the whole chip.
+// Cutting sequences and writing tokens need no plan. A table entry that names no page is met where the table is walked: a
+// fork passes it on, a cut drops it, a write skips it, and attention gives NaN.
 //
 // What bounds them: a plan is a few dependent passes over some thousand integers, so latency (37 sequences of one token 6.4
 // us, 16 prompts of up to 2304 tokens 9.2; forks 4.4 to 5.5 with 3.8 to 4.7 to carry them out, compactions 5.1 to 5.4, cuts 3.0
@@ -258,12 +259,12 @@ __global__ __launch_bounds__(256) void fork_apply_kernel(Cache c, const int32_t*
   for (int64_t t = threadIdx.x; t < n; t += 256) {
     const int p = from[t];
     const bool in = p >= 0 && p < c.n_pages;
-    if (copy) {
+    if (copy) {  // the page for an entry that names none stays free: copied onto itself
       const int at = w_off(c)[i] + (int)t, id = w_list(c)[at];
       w_src(c)[at] = in ? p : id;
       w_dst(c)[at] = id;
-      c.refs[id] = 1;
-      to[t] = id;
+      if (in) c.refs[id] = 1;
+      to[t] = in ? id : p;
     } else {
       if (in) atomicAdd(c.refs + p, 1);
       to[t] = p;

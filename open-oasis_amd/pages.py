@@ -16,7 +16,8 @@ from .kernels import check_heads, check_ints, launch
 
 REFUSALS = {L.PAGES_FULL: "too few free pages",
             L.PAGES_BAD_CALL: "a reserve or fork named a sequence that is not there, twice, or not empty, or too many tokens",
-            L.PAGES_BAD_ENTRY: "a truncate or write skipped a sequence, length, page or row that is not there"}
+            L.PAGES_BAD_ENTRY: "a truncate or write skipped a sequence, length, page or row that is not there, "
+                               "or a fork passed a page on that is not there"}
 
 
 class PageCache:

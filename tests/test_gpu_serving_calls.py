@@ -62,3 +62,37 @@ def test_a_write_of_fewer_rows_than_its_tokens_is_reported(bounds, rows):
     spare = torch.randn(20, 2, 64, device="cuda").to(BF)     # more rows than tokens are none of its business
     c.write(1, spare, -spare, ints([2, 0]), cumulated(counts))
     c.check()
+
+
+@pytest.mark.parametrize("bad", [-1, 40, 1 << 30])
+@pytest.mark.parametrize("copy", [False, True])
+def test_a_fork_passes_on_a_page_that_is_not_there(copy, bad):
+    """The child is what the parent is, that entry included, no page is lost on it, and check() names the call."""
+    c = new_cache()
+    m = Model(c)
+    extend(c, [0, 1], [70, 20], model=m)
+    was = m.tables[0][2]
+    c.tables[0, 2] = bad
+    c.fork(ints([0, 1]), ints([5, 3]), copy=copy)
+    m.fork([0, 1], [5, 3], copy)
+    m.refs[m.tables[5][2]] -= 1           # nobody is on the page that the entry would have named
+    m.tables[0][2] = m.tables[5][2] = bad
+    if copy:                              # nor is it copied to
+        lost = [p for p in range(40) if p not in m.tables[0] + m.tables[1] + m.tables[5] + m.tables[3] + [was]]
+        for pool, was_pool in ((m.k, c.k), (m.v, c.v)):
+            pool[:, lost] = was_pool[:, lost].cpu()
+    m.check(c)
+    with pytest.raises(L.OasisError, match="fork"):
+        c.check()
+    c.truncate(ints([5]))
+    assert int(c.status) == L.PAGES_BAD_ENTRY and int(c.lens[5]) == 0
+    with pytest.raises(L.OasisError):
+        c.check()
+    c.tables[0, 2] = was
+    m.tables[0][2] = was
+    m.tables[5][2] = was
+    m.refs[was] += 1
+    m.truncate([5], [0])
+    m.check(c)
+    assert extend(c, [5, 6, 7, 8, 9, 10, 11], [80] * 6 + [16 * (len(m.free()) - 30)], model=m) == 0     # all free pages can be had
+    m.check(c)
