@@ -500,7 +500,8 @@ int copy_pages(const Cache& c, int64_t most, int tables, hipStream_t s, const ch
 }  // namespace
 
 extern "C" int64_t oasis_pages_work(int64_t n_pages, int64_t max_seqs) {
-  if (n_pages <= 0 || max_seqs <= 0) return OASIS_ERR_SHAPE;
+  OASIS_REQUIRE(n_pages > 0 && max_seqs > 0, OASIS_ERR_SHAPE, "pages_work: %lld pages and %lld sequences", (long long)n_pages,
+                (long long)max_seqs);
   return W_LISTS + 3 * n_pages + 2 * max_seqs;
 }
 

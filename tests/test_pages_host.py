@@ -52,3 +52,10 @@ print("imported")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "imported" in r.stdout, r.stderr[-2000:]
+
+
+def test_scratch_sizes_that_are_refused_say_so():
+    for args in ((0, 7), (7, 0), (-1, 1)):
+        assert L.lib().oasis_pages_reserve(None, None, None, 1, None) < 0      # another message is the last
+        with pytest.raises(L.OasisError, match="%d pages and %d sequences" % args):
+            L.count("oasis_pages_work", *args)
