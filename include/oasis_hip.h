@@ -755,7 +755,7 @@ int oasis_video_decode(const oasis_dit_weights_t* w, const oasis_vae_weights_t* 
  *   sequence may be empty).
  *   out[r, h] = sum_j p_j v[j], p = softmax_j(scale q[r, h] . k[j]), over the rows j <= r of r's sequence.
  * out overlaps none of the others. Rows of no sequence are neither read nor written. A key or value counts for no row
- * before its own, be it infinite or NaN. total < 2^30, ld_k and ld_v < 2^24. */
+ * before its own, be it infinite or NaN. n <= 65536, total < 2^30, ld_k and ld_v < 2^24. */
 int oasis_prompt_attention(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
                            void* out, int64_t ld_out, const int32_t* cu, int64_t n, int64_t total, int64_t n_heads,
                            int64_t n_kv_heads, int64_t head_dim, float scale, oasis_stream_t stream);
@@ -800,7 +800,7 @@ int oasis_pages_reserve(const oasis_page_cache_t* cache, const int32_t* seqs, co
 /* The keys and values of the last cu[i+1] - cu[i] tokens of each sequence seqs[i], in one layer: rows cu[i] .. of k and v
  * [total, n_kv_heads, head_dim], ld_* elements apart (multiples of 8). Follows the reserve with the same seqs and cu.
  * Rows outside [cu[0], cu[n]) are not read. Tokens without a row (cu[0] < 0, cu[n] > total) are skipped, which sets
- * BAD_ENTRY; a call with total = 0 does nothing at all. */
+ * BAD_ENTRY; a call with total = 0 does nothing at all. total < 2^26. */
 int oasis_pages_write(const oasis_page_cache_t* cache, int64_t layer, const void* k, int64_t ld_k, const void* v,
                       int64_t ld_v, const int32_t* seqs, const int32_t* cu, int64_t n, int64_t total,
                       oasis_stream_t stream);

@@ -524,7 +524,7 @@ extern "C" int oasis_pages_write(const oasis_page_cache_t* cache, int64_t layer,
   if (const int rc = check_list(cache, seqs, n, "pages_write")) return rc;
   OASIS_REQUIRE(layer >= 0 && layer < cache->n_layers, OASIS_ERR_SHAPE, "pages_write: layer %lld of %lld", (long long)layer,
                 (long long)cache->n_layers);
-  OASIS_REQUIRE(total >= 0 && total < (1ll << 31), OASIS_ERR_SHAPE, "pages_write: bad token count");
+  OASIS_REQUIRE(total >= 0 && total < (1ll << 26), OASIS_ERR_SHAPE, "pages_write: bad token count");
   if (n == 0 || total == 0) return OASIS_OK;
   OASIS_REQUIRE(k && v && cu, OASIS_ERR_NULL, "pages_write: null pointer");
   const int64_t row = cache->n_kv_heads * cache->head_dim;

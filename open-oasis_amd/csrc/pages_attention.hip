@@ -831,8 +831,7 @@ template <int D>
 int pages_go(const PagesArgs& a, const Plan& p, hipStream_t s) {
   const int64_t hk = a.c.n_kv_heads, prefixes = p.p_tiles * hk * p.p_splits, per = NW / p.s_waves,
                 owns = (a.n_rows * hk * p.s_tiles * p.s_splits + per - 1) / per;
-  OASIS_REQUIRE(prefixes < (1ll << 31) && owns * per < (1ll << 31), OASIS_ERR_SHAPE, "pages_attention: too many parts");
-  OASIS_REQUIRE(prefixes + owns < (1ll << 31), OASIS_ERR_SHAPE, "pages_attention: too many parts");
+  OASIS_REQUIRE((prefixes + owns) * NW * 64 < (1ll << 32), OASIS_ERR_SHAPE, "pages_attention: too many parts");  // one launch's threads
   if (p.at_once) {
     const auto fn = p.p_waves == 8 ? &both_kernel<D, 8> : &both_kernel<D, 1>;
     hipLaunchKernelGGL(fn, dim3((unsigned)(prefixes + owns)), dim3(NW * 64), 0, s, a, (int)prefixes);

@@ -145,7 +145,7 @@ template <int D>
 int prompt_go(PromptArgs a, int64_t heads, int hg, hipStream_t s) {
   a.hblocks = (int)(heads / hg);
   const int64_t span = 32 * NW / hg, tiles = a.total / span + std::min<int64_t>(a.n, a.total);
-  OASIS_REQUIRE(tiles * a.hblocks < (1ll << 31), OASIS_ERR_SHAPE, "prompt_attention: too many query tiles");
+  OASIS_REQUIRE(tiles * a.hblocks * NW * 64 < (1ll << 32), OASIS_ERR_SHAPE, "prompt_attention: too many query tiles");
   hipLaunchKernelGGL((prompt_kernel<D>), dim3((unsigned)(tiles * a.hblocks)), dim3(NW * 64), 0, s, a, hg);
   return oasis::check_launch("prompt_attention");
 }
@@ -158,7 +158,7 @@ extern "C" int oasis_prompt_attention(const void* q, int64_t ld_q, const void* k
   OASIS_REQUIRE(head_dim == 64 || head_dim == 128, OASIS_ERR_SHAPE, "prompt_attention: head_dim must be 64 or 128");
   OASIS_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads <= 4096 && n_heads % n_kv_heads == 0, OASIS_ERR_SHAPE,
                 "prompt_attention: n_heads must be a multiple of n_kv_heads, up to 4096");
-  OASIS_REQUIRE(n >= 0 && total >= 0 && n < (1ll << 24) && total < (1ll << 30), OASIS_ERR_SHAPE,
+  OASIS_REQUIRE(n >= 0 && total >= 0 && n <= 65536 && total < (1ll << 30), OASIS_ERR_SHAPE,
                 "prompt_attention: bad sequence or token count");
   OASIS_REQUIRE(scale > 0 && scale < INFINITY, OASIS_ERR_ARG, "prompt_attention: the scale must be positive and finite");
   if (n == 0 || total == 0) return OASIS_OK;

@@ -1,4 +1,5 @@
 """What the Python surface of prompts and cache pages refuses or takes on the host, before any device work."""
+import ctypes
 import os
 import subprocess
 import sys
@@ -59,3 +60,29 @@ def test_scratch_sizes_that_are_refused_say_so():
         assert L.lib().oasis_pages_reserve(None, None, None, 1, None) < 0      # another message is the last
         with pytest.raises(L.OasisError, match="%d pages and %d sequences" % args):
             L.count("oasis_pages_work", *args)
+
+
+FAKE = ctypes.c_void_p(0x1000)
+SHAPE = -2
+
+
+def cache(**kw):
+    a = dict(k=16, v=16, refs=16, tables=16, lens=16, status=16, work=16, n_layers=2, n_pages=10, page_size=16, n_kv_heads=2, head_dim=64,
+             max_seqs=65536, max_pages=8) | kw
+    return ctypes.byref(L.PageCache(*a.values()))
+
+
+@pytest.mark.parametrize("name,args,needle", [
+    ("oasis_prompt_attention", (FAKE, 64, FAKE, 64, FAKE, 64, FAKE, 64, FAKE, 65537, 1 << 20, 1, 1, 64, 0.1, None), "count"),
+    # 2^16 + 2^12 tiles of 128 heads, more than one launch has
+    ("oasis_prompt_attention", (FAKE, 8192, FAKE, 8192, FAKE, 8192, FAKE, 8192, FAKE, 65536, 1 << 20, 128, 128, 64, 0.1, None), "tiles"),
+    ("oasis_pages_write", (cache(), 0, FAKE, 128, FAKE, 128, FAKE, FAKE, 1, 1 << 26, None), "count"),
+    ("oasis_pages_attention", (cache(n_kv_heads=1024), 0, FAKE, 65536, FAKE, 65536, FAKE, 65536, None, None, 0, 5000, 1024, 0.1, FAKE, 1 << 40,
+                               None), "parts"),
+    ("oasis_pages_attention", (cache(n_kv_heads=1024), 0, FAKE, 65536, FAKE, 65536, FAKE, 65536, FAKE, FAKE, 60000, 5000, 1024, 0.1, FAKE,
+                               1 << 50, None), "parts")])
+def test_calls_of_more_workgroups_than_a_launch_has_are_refused(name, args, needle):
+    """A launch has less than 2^32 threads."""
+    h = L.lib()
+    rc = getattr(h, name)(*args)
+    assert rc == SHAPE and needle in h.oasis_last_error().decode(), (rc, h.oasis_last_error())
