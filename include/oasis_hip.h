@@ -793,7 +793,8 @@ int64_t oasis_pages_work(int64_t n_pages, int64_t max_seqs);
 
 /* Room for cu[i+1] - cu[i] more tokens of each sequence seqs[i], i < n (distinct): its length grows and free pages, the
  * lowest numbers first, in order, join its table. A part-filled last page that other sequences share is first
- * replaced by a copy. seqs and cu on the device. */
+ * replaced by a copy; so for every sharer that the call names, which takes one page more than leaving it to the last of them
+ * where all are named. seqs and cu on the device. */
 int oasis_pages_reserve(const oasis_page_cache_t* cache, const int32_t* seqs, const int32_t* cu, int64_t n,
                         oasis_stream_t stream);
 
@@ -827,6 +828,9 @@ int oasis_pages_compact(const oasis_page_cache_t* cache, oasis_stream_t stream);
  *   first row, and as far as that has tokens. Rows of no group, and all with n_groups = 0, read everything through their own.
  *   out[r, h] = sum_j p_j v[j], p = softmax_j(scale q[r, h] . k[j]), over all tokens of the sequence; 0 where it has none,
  *   NaN where seqs[r] is no sequence or a table names a page that is not there.
+ *   n_groups: of groups that have rows. What is read together is decided on the host by the counts alone, for groups of about
+ *   the same size: with n_groups >= n_rows every row reads everything itself, so empty groups behind the others (which the
+ *   device's bounds allow) cost the sharing, or part of it, and no more than that. out overlaps none of the others.
  *   max_len: about how many tokens the longest sequence has (it sizes the split of long ones; longer ones are right, and
  *   slower). workspace: oasis_pages_attention_workspace bytes (for the same or larger counts), 16-byte aligned; calls that
  *   share it must not overlap. seqs, cu_groups and prefix_lens on the device. */

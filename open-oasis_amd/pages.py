@@ -58,7 +58,7 @@ class PageCache:
 
     def reserve(self, seqs, cu):
         """Room for the new tokens of seqs (distinct): lengths grow, the lowest free pages join the tables, a part-filled
-        last page that others share is replaced by a copy."""
+        last page that others share is replaced by a copy, for each of them that is named."""
         self._lists("reserve", seqs, cu)
         launch(self._dev, "oasis_pages_reserve", self._ref, seqs.data_ptr(), cu.data_ptr(), seqs.numel())
 
@@ -105,7 +105,9 @@ def make_prefix_attention_kernel(cache, n_heads, scale_val, max_rows, max_groups
 
     The kernel takes layer, q [rows, n_heads, head_dim] (bf16), seqs [rows], cu_groups [groups + 1] and prefix_lens
     [groups] (rows cu_groups[g] .. cu_groups[g + 1] - 1 begin with the same prefix_lens[g] tokens; None for both where
-    nothing is shared), and out like q. max_len: about how many tokens the longest sequence has.
+    nothing is shared), and out like q, which overlaps none of them. max_len: about how many tokens the longest sequence has.
+    The prefixes are read together where there are fewer groups than rows, whatever the groups' bounds are: groups without
+    rows, as in vectors padded to a fixed size, give right results and cost the sharing.
 
     The workspace is the kernel's own: its calls must not overlap, nor graphs that hold them."""
     work = L.count("oasis_pages_attention_workspace", max_rows, max_groups, max_len, n_heads, cache.n_kv_heads,
