@@ -594,6 +594,9 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, WaveSum (*wml
       scores(t);
       look(t + S);
       load_k();
+      // weigh's wait counts these loads as the last before it: none may sink past it (nor rise past this tile's values, which
+      // were loaded in the round before); what is not a load from memory may
+      __builtin_amdgcn_sched_barrier(0x38F);
       weigh(std::true_type());
       __builtin_amdgcn_s_waitcnt(0xF | (3 << 14) | (0x7 << 4));  // lgkmcnt(0): the values are read before they are loaded over
       load_v();
