@@ -550,7 +550,10 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, WaveSum (*wml
     const float alpha = __builtin_amdgcn_exp2f(flash::shift(was, base, a.scale_log2));
     was = base;
     m = to;
-    bf16x8 pb;  // rounded for the product, as flash::Tile::probs
+    // Rounded for the product, as flash::Tile::probs. Here the matrix units have time, but not the registers: with a second
+    // product for what the rounding leaves, 256 rows of up to 1000 tokens of 8 key heads of 128 take 126 us for 102 (16 key
+    // heads of 64, up to 180 tokens: 23.9 for 23.7), and the prefixes' parts of a row are rounded like this anyway.
+    bf16x8 pb;
     float sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
