@@ -799,8 +799,18 @@ Plan plan_of(int64_t n_rows, int64_t n_groups, int64_t max_len, int64_t group, i
   // 128, take 40, 74 and 150 us this way and 58, 108 and 212 in parts.
   if (n_groups >= n_rows) n_groups = 0;
   const int64_t cols = n_groups ? n_rows * group / n_groups : 0;  // of a group, on the average
-  // Few columns: behind 40000 shared tokens, heads of 128, 60 columns take 48.5 us with R = 1 and 51.1 with 8, 80 take 54.4
-  // and 51.2; heads of 64, 80 take 57.9 and 70.4, 130 take 86 and 77. (R = 2 was between the two or behind both.)
+  // Few columns or many. One group of 8 key heads, us with R = 1 and with 8:
+  //   columns of 128    2000 tokens shared   16000         40000
+  //    80               15.2, 20.7           26.9, 30.1    54.6, 51.2
+  //   240               25.0, 28.1           43.3, 46.3    94.2, 71.7
+  //   480               34.8, 29.4           71.4, 67.1   153.6, 108.0
+  //   columns of 64
+  //    80               12.0, 16.7           18.1, 24.4    27.0, 34.9
+  //   132               12.8, 20.9           21.6, 31.8    36.7, 45.8
+  //   240               17.2, 22.7           27.2, 34.8    52.1, 50.3
+  //   480               21.2, 24.6           41.5, 52.3    92.6, 81.5
+  // The border is that of long prefixes; behind shorter ones R = 8 is taken too early, by up to 11 us. (R = 2 was between the two
+  // or behind both.)
   p.p_waves = cols * D > 8192 ? 8 : 1;
   p.p_tiles = n_groups ? n_rows * group / (32 * p.p_waves) + n_groups : 0;
   // A part to each CU: the four groups of the kernels' comment take 181 us, 198 with 128 parts, 192 with 384, 200 with 512.
