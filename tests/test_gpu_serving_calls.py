@@ -96,3 +96,49 @@ def test_a_fork_passes_on_a_page_that_is_not_there(copy, bad):
     m.check(c)
     assert extend(c, [5, 6, 7, 8, 9, 10, 11], [80] * 6 + [16 * (len(m.free()) - 30)], model=m) == 0     # all free pages can be had
     m.check(c)
+
+
+def test_calls_of_more_sequences_than_a_workgroup_plans_at_a_time():
+    """Writes that search bounds in memory (1024 sequences on), forks of more than one pass (1024), copies of part-filled pages by
+    lists in memory (2048 on): each against the model, in full."""
+    import random
+    r = random.Random(8)
+    c = pkg.PageCache(1, 9001, 16, 1, 64, 2500, 4)
+    c.k.zero_()
+    c.v.zero_()
+    m = Model(c)
+    parents = r.sample(range(1300), 1300)
+    assert extend(c, parents, [r.choice([0, 1, 5, 16, 33]) for _ in parents], seed=1, model=m) == 0
+    m.check(c)
+    kids = r.sample(range(1300, 2500), 1200)
+    of = [r.randrange(1300) for _ in kids]
+    c.fork(ints(of), ints(kids))
+    assert m.fork(of, kids, False) == 0
+    m.check(c)
+    grow = r.sample(range(2500), 2300)
+    assert extend(c, grow, [r.choice([0, 1, 1, 2]) for _ in grow], seed=2, model=m) == 0
+    m.check(c)
+    c.truncate(ints(kids))
+    m.truncate(kids, [0] * len(kids))
+    c.fork(ints(of), ints(kids), copy=True)
+    assert m.fork(of, kids, True) == 0
+    m.check(c)
+    c.compact()
+    m.compact()
+    m.check(c)
+    c.check()
+
+
+def test_attention_over_pages_past_32_bits():
+    """A layer of 5 GB: own tokens and prefixes of few and of many columns on its last pages, in the second layer."""
+    c = pkg.PageCache(2, 40000, 64, 8, 128, 6, 19600)
+    c.reserve(ints([0, 1]), ints([0, 39000 * 32, 39000 * 64]))
+    extend(c, [2], [300])
+    c.fork(ints([2, 2]), ints([3, 4]))
+    extend(c, [2, 3, 4, 5], [5, 70, 1, 90], seed=1)
+    c.check()
+    assert int(c.tables[2:, 0].min()) >= 39000
+    check_attention(c, 8, [2, 3, 4, 5], layer=1, max_len=400)
+    for heads in (8, 192):
+        check_attention(c, heads, [2, 3, 4, 5], [0, 3, 4], [256, 60], layer=1, max_len=400)
+    check_attention(c, 8, [5, 2], layer=0, max_len=400)
