@@ -16,6 +16,7 @@ typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 
 namespace flash {
 
+constexpr int NW = 8;  // waves of a workgroup
 constexpr float LOG2E = 1.4426950408889634f;
 // How far a row's scores may pass its running maximum before the sums are rescaled, as a power of two: the probabilities
 // reach 2^8 then, which costs neither bf16 nor fp32 any precision.
@@ -255,7 +256,7 @@ struct Tile {
 template <int D>
 struct Turns {
   typedef Tile<D> Tile;
-  static constexpr int NW = 8, KS = 64, ROW = Tile::ROW, HALF = KS * ROW, STAGE = 2 * HALF, ST = 4, SMEM = ST * STAGE;
+  static constexpr int KS = 64, ROW = Tile::ROW, HALF = KS * ROW, STAGE = 2 * HALF, ST = 4, SMEM = ST * STAGE;
   static constexpr int RPB = 1024 / ROW;         // rows of a 1 KB load
   static constexpr int LPW = 2 * KS / RPB / NW;  // loads of a wave and stage: rows [16 (wave % 4), + 16) of the keys (the
                                                  // first four waves) or the values

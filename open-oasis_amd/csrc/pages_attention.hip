@@ -51,7 +51,7 @@ struct PagesArgs {
   Sum* ml;    // [rows][heads][parts]
 };
 
-constexpr int NW = 8;
+using flash::NW;
 constexpr int MIN_CHUNK = 256;  // keys of a part at least: a tile of 32 for every wave, two where it is a row's own
 
 // keys of each of `splits` parts of n
@@ -206,7 +206,6 @@ struct Walk {
 #pragma unroll
       for (int s = 0; s < Tile::DS; ++s) w.q[s] = *reinterpret_cast<const bf16x8*>(qp + 16 * s);
     }
-    constexpr int N = KT / 32;
     auto leave = [&](int it) {
       const int t = it * S + wave;
       if (t + S < n) {
@@ -226,19 +225,12 @@ struct Walk {
           if (key >= k1) *reinterpret_cast<f32x4*>(vb + x * 16) = f32x4{0.f, 0.f, 0.f, 0.f};
         }
       if (t < n) {
-        f32x16 s[N];
+        f32x16 s = w.scores(kb, lane);
 #pragma unroll
-        for (int c = 0; c < N; ++c) {
-          s[c] = w.scores(kb + c * 32 * ROW, lane);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = key0 + c * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-            if (key >= min(k1, end)) s[c][i] = -INFINITY;
-          }
-        }
-        w.template softmax<N>(s, a.scale_log2);
-#pragma unroll
-        for (int c = 0; c < N; ++c) w.weigh(s[c], vb + c * 32 * ROW, lane);
+        for (int i = 0; i < 16; ++i)
+          if (key0 + 8 * (i >> 2) + 4 * h + (i & 3) >= min(k1, end)) s[i] = -INFINITY;
+        w.template softmax<1>(&s, a.scale_log2);
+        w.weigh(s, vb, lane);
       }
       leave(it);
     };
@@ -255,12 +247,9 @@ struct Walk {
     while (it < plain) {
       __builtin_amdgcn_s_waitcnt(0);
       const char *kb = stage, *vb = stage + HALF;
-      f32x16 s[N];
-#pragma unroll
-      for (int c = 0; c < N; ++c) s[c] = w.scores(kb + c * 32 * ROW, lane);
-      w.template softmax<N>(s, a.scale_log2);
-#pragma unroll
-      for (int c = 0; c < N; ++c) w.weigh(s[c], vb + c * 32 * ROW, lane);
+      f32x16 s = w.scores(kb, lane);
+      w.template softmax<1>(&s, a.scale_log2);
+      w.weigh(s, vb, lane);
       leave(it++);
     }
 #pragma unroll 1

@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int NW = 8;  // waves of a workgroup
+using flash::NW;
 
 struct PromptArgs {
   const bf16 *q, *k, *v;
