@@ -123,3 +123,48 @@ def test_prompts(raws, d):
         torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -float("inf"))
     p = s.softmax(-1)
     check(out[:, 0], p @ v[:, 0].double(), p @ v[:, 0].double().abs())
+
+
+def below(n, raws, d, seed):
+    """Keys whose scores all lie far below zero, up to 400 apart, and values of both signs."""
+    g = torch.Generator().manual_seed(seed)
+    raw = torch.randint(raws[0], raws[1], (1,), generator=g) + torch.randint(0, 401, (n,), generator=g)
+    k = torch.zeros(n, d)
+    k[:, 0], k[:, 1], k[:, 2] = raw >> 16, raw >> 8 & 255, raw & 255    # as key_of
+    return k.to(BF).cuda(), (torch.randint(0, 2, (n,), generator=g) * 2 - 1).to(BF).cuda()
+
+
+@pytest.mark.parametrize("raws", RAW)
+@pytest.mark.parametrize("rows,hk,heads,d,shared", [(3, 1, 1, 64, False), (64, 16, 16, 128, False), (4, 1, 2, 64, True), (40, 1, 4, 128, True),
+                                                    (600, 16, 16, 64, True)])
+def test_scores_far_below_zero(rows, hk, heads, d, shared, raws):
+    r = random.Random(rows)
+    if shared:
+        prefix = [16 * r.randint(19, 43) for _ in range(2)]
+        c, cu = branches(prefix, [[r.randint(2, 40) for _ in range(rows // 2)] for _ in prefix], 16, hk, d)
+    else:
+        prefix, cu = None, None
+        c = filled([r.randint(400, 800) for _ in range(rows)], 16, hk, d)
+    k, v = below(c.refs.numel() * 16, raws, d, rows + raws[0])
+    c.k[0] = k.view(-1, 1, 16, d)
+    c.v[0] = v.view(-1, 1, 16, 1)
+    q = -query(rows, heads, d)
+    out = torch.zeros_like(q)
+    f = pkg.make_prefix_attention_kernel(c, heads, SCALE, rows, len(prefix) if prefix else 0, int(c.lens.max()))
+    f(0, q, ints(list(range(rows))), cu and ints(cu), prefix and ints(prefix), out)
+    check(out, *reference(c, 0, q, range(rows), SCALE))
+
+
+@pytest.mark.parametrize("raws", RAW)
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompts_of_scores_far_below_zero(raws, d):
+    n = 700
+    k, v = below(n, raws, d, d + raws[0])
+    q = -query(n, 1, d)
+    v = v.view(n, 1, 1).expand(n, 1, d).contiguous()
+    out = torch.zeros_like(q)
+    pkg.kernels.make_prompt_attention_kernel(1, 1, d, SCALE)(q, k.view(n, 1, d), v, ints([0, n]), out)
+    s = (q[:, 0].double() @ k.double().t().contiguous() * SCALE).masked_fill(
+        torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -float("inf"))
+    p = s.softmax(-1)
+    check(out[:, 0], p @ v[:, 0].double(), p @ v[:, 0].double().abs())
