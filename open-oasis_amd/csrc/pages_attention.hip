@@ -12,8 +12,8 @@
 //
 // What bounds it: own tokens are read once, which is bandwidth (256 rows of up to 1024 tokens, 8 key heads of 128, 545 MB: 116
 // us, 4.7 TB/s); a prefix of many columns the products on tiles of 256 columns (256 rows in four groups, prefixes of up to
-// 16000 tokens, 32 heads of 128, 8 key heads, with their own tokens up to 1024: 178 us); few rows the latency of loads
-// behind each other and of two launches (one row of 720 tokens, 16 heads of 64: 7.4 us; 32 rows behind 4608 shared ones: 15.3).
+// 16000 tokens, 32 heads of 128, 8 key heads, with their own tokens up to 1024: 180 us); few rows the latency of loads
+// behind each other and of two launches (one row of 720 tokens, 16 heads of 64: 7.4 us; 32 rows behind 4608 shared ones: 16.0).
 #include <algorithm>
 #include <type_traits>
 

@@ -7,7 +7,7 @@
 //
 // What bounds it: the softmax of a tile takes the vector units about as long as its products take the matrix units (D = 128:
 // 190 vector instructions and 32 products of 32 cycles to a wave and tile; D = 64: the same and 16), so the waves of a SIMD
-// take turns at them, kept in step by barriers. 8192 tokens, 32 heads of 128, 8 key heads: 470 to 490 us over runs, 1.12 to
+// take turns at them, kept in step by barriers. 8192 tokens, 32 heads of 128, 8 key heads: 470 to 494 us over runs, 1.11 to
 // 1.17 PFLOP/s (a library product of 8192^3 reaches 1.21); before the waves took turns 533. 8192 tokens, 16 heads of 64: 160
 // us, 0.86 PFLOP/s.
 #include <algorithm>
