@@ -537,7 +537,7 @@ OASIS_DEV void own_part(const PagesArgs& a, int block, char* smem, WaveSum (*wml
     const float to = fmaxf(m, mx);
     const flash::Base base = top_base(to, a.scale_log2);
     const float alpha = __builtin_amdgcn_exp2f(flash::shift(was, base, a.scale_log2));
-    was = base;
+    was = flash::Base{to == -INFINITY ? to : base.raw, base.number};  // nothing is taken on a base yet where no score is a number
     m = to;
     // Rounded for the product, as flash::Tile::probs. Here the matrix units have time, but not the registers: with a second
     // product for what the rounding leaves, 256 rows of up to 1000 tokens of 8 key heads of 128 take 126 us for 102 (16 key

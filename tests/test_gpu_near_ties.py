@@ -168,3 +168,51 @@ def test_prompts_of_scores_far_below_zero(raws, d):
         torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -float("inf"))
     p = s.softmax(-1)
     check(out[:, 0], p @ v[:, 0].double(), p @ v[:, 0].double().abs())
+
+
+@pytest.mark.parametrize("rows,hk,heads,d,lens,shared", [(300, 4, 4, 64, 60, 0), (3, 1, 1, 128, 700, 0), (64, 16, 16, 64, 500, 0), (4, 1, 2, 64, 320, 304),
+                                                         (40, 1, 4, 128, 320, 304)])
+@pytest.mark.parametrize("gone", [32, 256])
+def test_keys_of_minus_infinity_before_scores_far_below_zero(rows, hk, heads, d, lens, shared, gone):
+    """Whole tiles that count for nothing, and behind them a row's first finite scores."""
+    gone = min(gone, 32 if lens < 300 else 256)
+    if shared:
+        c, cu = branches([shared], [[lens - shared] * rows], 16, hk, d)
+    else:
+        c, cu = filled([lens] * rows, 16, hk, d), None
+    g = torch.Generator(device="cuda").manual_seed(1)
+    c.v.copy_(torch.randn(c.v.shape, generator=g, device="cuda").to(BF))
+    c.k.zero_()
+    c.k[..., 0] = (torch.randn(c.k.shape[:-1], generator=g, device="cuda") - 3000).to(BF)
+    pages = c.tables[:, :gone // 16].flatten().unique().long()
+    c.k[:, pages, :, :, 0] = -float("inf")
+    q = torch.zeros(rows, heads, d, dtype=BF, device="cuda")
+    q[..., 0] = 1
+    out = torch.zeros_like(q)
+    f = pkg.make_prefix_attention_kernel(c, heads, SCALE, rows, 1 if shared else 0, lens)
+    f(0, q, ints(list(range(rows))), ints([0, rows]) if shared else None, ints([shared]) if shared else None, out)
+    n = torch.arange(lens, device="cuda")
+    for row in (0, rows - 1):
+        ids = c.tables[row].long()[n // 16]
+        for h in range(heads):
+            s = c.k[0, ids, h * hk // heads, n % 16, 0].double() * SCALE
+            p, v = s.softmax(0), c.v[0, ids, h * hk // heads, n % 16].double()
+            check(out[row, h], p @ v, p @ v.abs())
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompts_whose_last_keys_score_minus_infinity(d):
+    n = 400
+    g = torch.Generator().manual_seed(2)
+    k, v, q = (torch.zeros(n, 1, d) for _ in range(3))
+    k[:, 0, 0], q[:, 0, 0] = torch.randn(n, generator=g) - 3000, 1
+    k[130:, 0, 0] = -float("inf")
+    v.copy_(torch.randn(n, 1, d, generator=g))
+    q, k, v = (x.to(BF).cuda() for x in (q, k, v))
+    out = torch.zeros_like(q)
+    pkg.kernels.make_prompt_attention_kernel(1, 1, d, SCALE)(q, k, v, ints([0, n]), out)
+    s = (k[:, 0, 0].double() * SCALE).expand(n, n).masked_fill(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -float("inf"))
+    p = s.softmax(-1)
+    check(out[:, 0], p @ v[:, 0].double(), p @ v[:, 0].double().abs())
+    assert torch.isfinite(out).all()
