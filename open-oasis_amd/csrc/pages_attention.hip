@@ -13,7 +13,7 @@
 // What bounds it: own tokens are read once, which is bandwidth (256 rows of up to 1024 tokens, 8 key heads of 128, 545 MB: 116
 // us, 4.7 TB/s); a prefix of many columns the products on tiles of 256 columns (256 rows in four groups, prefixes of up to
 // 16000 tokens, 32 heads of 128, 8 key heads, with their own tokens up to 1024: 180 us); few rows the latency of loads
-// behind each other and of two launches (one row of 720 tokens, 16 heads of 64: 7.4 us; 32 rows behind 4608 shared ones: 16.0).
+// behind each other and of two launches (one row of 720 tokens, 16 heads of 64: 7.4 us; 32 rows behind 4608 shared ones: 15.7).
 #include <algorithm>
 #include <type_traits>
 
@@ -259,6 +259,10 @@ struct Walk {
 
     // The waves' sums. Lane l of every wave holds the same column's outputs; each wave joins its share.
     const int keys = max(min(k1, end) - k0, 0);  // that this lane's column sees
+    // the column's row and head once more: kept over the loops they go to scratch (32 branches 15.9 us, 15.6 this way)
+    int again = lr;
+    asm volatile("" : "+v"(again));
+    const int flat2 = pt.col0 + min(again, pt.cols - 1), row2 = pt.base_row + flat2 / a.group, head2 = pt.kvh * a.group + flat2 % a.group;
     if (bad) *missing = 1;
     __syncthreads();  // every wave is done with its stage, and has said whether it met a page that is not there
     const float lsum = *missing ? NAN : sum_xor32(w.l);
@@ -293,7 +297,7 @@ struct Walk {
     }
     if (lr >= pt.cols) return;
     if (m == -INFINITY && l == 0.f && keys > 0) l = -1.f;  // no probability is a number, which is not an empty row
-    const int64_t slot = ((int64_t)row * a.heads + head) * a.parts + pt.part;
+    const int64_t slot = ((int64_t)row2 * a.heads + head2) * a.parts + pt.part;
 #pragma unroll
     for (int r = 0; r < SHARE; r += 4) {
       const int g = wave * SHARE + r;  // dims 32 dt + 8 b + 4 h
