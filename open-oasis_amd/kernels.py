@@ -41,14 +41,33 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torc
 
 
 def launch(device, name, *args):
-    """L.call on the current stream of a device (its number), which is made the current device where it is not."""
+    """L.call on the current stream of a device (its number), which is made the current device where it is not. Returns the
+    stream's handle."""
     if device < 0:
         raise L.OasisError(name, -5, "expected device tensors, got some in host memory")
+    stream = _raw_stream(device)
     if torch.cuda.current_device() != device:
         with torch.cuda.device(device):
-            L.call(name, *args, _raw_stream(device))
+            L.call(name, *args, stream)
     else:
-        L.call(name, *args, _raw_stream(device))
+        L.call(name, *args, stream)
+    return stream
+
+
+class Streams:
+    """The streams that use memory which no caller holds: it is given out again when they are done with it, not only the one
+    that it was allocated on."""
+
+    def __init__(self, device, *tensors):
+        self.device, self.tensors = device, tensors
+        self.seen = {_raw_stream(device)} if device >= 0 else set()
+
+    def used(self, stream):
+        """A call went to a stream, the current one (its handle)."""
+        if stream not in self.seen:
+            self.seen.add(stream)
+            for t in self.tensors:
+                t.record_stream(torch.cuda.current_stream(self.device))
 
 
 def check_heads(what, t, rows, heads, head_dim, device):

@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib as L
-from .kernels import check_heads, check_ints, launch
+from .kernels import Streams, check_heads, check_ints, launch
 
 REFUSALS = {L.PAGES_FULL: "too few free pages",
             L.PAGES_BAD_CALL: "a reserve or fork named a sequence that is not there, twice, or not empty, or too many tokens",
@@ -50,6 +50,10 @@ class PageCache:
         self.struct = L.PageCache(*p, *sizes)
         self._ref = ctypes.byref(self.struct)
         self._dev = self.refs.get_device()
+        self._streams = Streams(self._dev, self.k, self.v, self.refs, self.tables, self.lens, self.status, self._work)
+
+    def _launch(self, name, *args):
+        self._streams.used(launch(self._dev, name, self._ref, *args))
 
     def _lists(self, what, seqs, cu):
         check_ints(what, self._dev, seqs, cu)
@@ -60,7 +64,7 @@ class PageCache:
         """Room for the new tokens of seqs (distinct): lengths grow, the lowest free pages join the tables, a part-filled
         last page that others share is replaced by a copy, for each of them that is named."""
         self._lists("reserve", seqs, cu)
-        launch(self._dev, "oasis_pages_reserve", self._ref, seqs.data_ptr(), cu.data_ptr(), seqs.numel())
+        self._launch("oasis_pages_reserve", seqs.data_ptr(), cu.data_ptr(), seqs.numel())
 
     def write(self, layer, k, v, seqs, cu):
         """The keys and values [rows, n_kv_heads, head_dim] of the tokens reserved last with the same seqs and cu."""
@@ -68,8 +72,8 @@ class PageCache:
         rows = k.shape[0]
         ld_k = check_heads("write", k, rows, self.n_kv_heads, self.head_dim, self._dev)
         ld_v = check_heads("write", v, rows, self.n_kv_heads, self.head_dim, self._dev)
-        launch(self._dev, "oasis_pages_write", self._ref, layer, k.data_ptr(), ld_k, v.data_ptr(), ld_v,
-               seqs.data_ptr(), cu.data_ptr(), seqs.numel(), rows)
+        self._launch("oasis_pages_write", layer, k.data_ptr(), ld_k, v.data_ptr(), ld_v, seqs.data_ptr(), cu.data_ptr(),
+                     seqs.numel(), rows)
 
     def fork(self, parents, children, copy=False):
         """Each empty sequence children[i] (distinct) becomes what parents[i] is, on the same pages, or with copy on free
@@ -77,19 +81,18 @@ class PageCache:
         check_ints("fork", self._dev, parents, children)
         if parents.numel() != children.numel():
             raise L.OasisError("fork", -2, "%d parents and %d children" % (parents.numel(), children.numel()))
-        launch(self._dev, "oasis_pages_fork", self._ref, parents.data_ptr(), children.data_ptr(), parents.numel(), bool(copy))
+        self._launch("oasis_pages_fork", parents.data_ptr(), children.data_ptr(), parents.numel(), bool(copy))
 
     def truncate(self, seqs, keep=None):
         """Cuts seqs to their first keep[i] tokens (none by default); pages that no sequence is left on become free."""
         check_ints("truncate", self._dev, seqs, *(() if keep is None else (keep,)))
         if keep is not None and keep.numel() != seqs.numel():
             raise L.OasisError("truncate", -2, "%d sequences and %d lengths" % (seqs.numel(), keep.numel()))
-        launch(self._dev, "oasis_pages_truncate", self._ref, seqs.data_ptr(), None if keep is None else keep.data_ptr(),
-               seqs.numel())
+        self._launch("oasis_pages_truncate", seqs.data_ptr(), None if keep is None else keep.data_ptr(), seqs.numel())
 
     def compact(self):
         """Moves the pages in use to the lowest numbers; tables and references follow."""
-        launch(self._dev, "oasis_pages_compact", self._ref)
+        self._launch("oasis_pages_compact")
 
     def check(self):
         """Waits for the calls so far; raises OasisError if one was refused, and clears the refusal."""
@@ -109,12 +112,14 @@ def make_prefix_attention_kernel(cache, n_heads, scale_val, max_rows, max_groups
     The prefixes are read together where there are fewer groups than rows, whatever the groups' bounds are: groups without
     rows, as in vectors padded to a fixed size, give right results and cost the sharing.
 
-    The workspace is the kernel's own: its calls must not overlap, nor graphs that hold them."""
+    The workspace is the kernel's own: its calls must not overlap, nor graphs that hold them, which need it as long as they
+    are replayed."""
     work = L.count("oasis_pages_attention_workspace", max_rows, max_groups, max_len, n_heads, cache.n_kv_heads,
                    cache.head_dim)
     workspace = torch.empty(work, dtype=torch.uint8, device=cache.device)
 
     dev, dim, at = cache._dev, cache.head_dim, workspace.data_ptr()
+    streams = Streams(dev, workspace)
 
     def prefix_attention_kernel(layer, q, seqs, cu_groups, prefix_lens, out):
         if (cu_groups is None) != (prefix_lens is None):
@@ -132,7 +137,9 @@ def make_prefix_attention_kernel(cache, n_heads, scale_val, max_rows, max_groups
         if seqs.numel() != rows or rows > max_rows or groups > max_groups:
             raise L.OasisError("prefix_attention", -2, "%d rows of %d sequences in %d groups; the kernel was made for %d and %d"
                                % (rows, seqs.numel(), groups, max_rows, max_groups))
-        launch(dev, "oasis_pages_attention", cache._ref, layer, q.data_ptr(), ld_q, out.data_ptr(), ld_out,
-               seqs.data_ptr(), rows, cu_groups.data_ptr() if groups else None, prefix_lens.data_ptr() if groups else None,
-               groups, max_len, n_heads, scale_val, at, workspace.numel())
+        stream = launch(dev, "oasis_pages_attention", cache._ref, layer, q.data_ptr(), ld_q, out.data_ptr(), ld_out,
+                        seqs.data_ptr(), rows, cu_groups.data_ptr() if groups else None,
+                        prefix_lens.data_ptr() if groups else None, groups, max_len, n_heads, scale_val, at, workspace.numel())
+        streams.used(stream)
+        cache._streams.used(stream)
     return prefix_attention_kernel

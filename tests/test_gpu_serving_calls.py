@@ -142,3 +142,48 @@ def test_attention_over_pages_past_32_bits():
     for heads in (8, 192):
         check_attention(c, heads, [2, 3, 4, 5], [0, 3, 4], [256, 60], layer=1, max_len=400)
     check_attention(c, 8, [5, 2], layer=0, max_len=400)
+
+
+def overlaps(span, like):
+    """Whether the allocator gives out any of the memory [first, last) for tensors of a size."""
+    got = [torch.empty_like(like) for _ in range(8)]
+    return any(t.data_ptr() < span[1] and span[0] < t.data_ptr() + t.numel() * t.element_size() for t in got)
+
+
+def busy(stream):
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)    # some tenths of a second
+
+
+def test_memory_of_a_kernel_or_cache_dropped_while_another_stream_uses_it_is_not_given_out():
+    """As for any tensor that its stream has been told of: the workspace is nobody's to tell of but the kernel's."""
+    c, cu = branches([300], [[3, 50, 7, 0]], 16, 2, 64)
+    side = torch.cuda.Stream()
+    q = torch.randn(4, 4, 64, device="cuda").to(BF)
+    out = torch.zeros_like(q)
+    args = ints(range(4)), ints(cu), ints([300])
+    torch.cuda.synchronize()
+    f = pkg.make_prefix_attention_kernel(c, 4, 0.125, 4, 1, 400)
+    workspace = next(x.cell_contents for x in f.__closure__ if torch.is_tensor(x.cell_contents))
+    like, span = torch.empty_like(workspace, device="meta"), (workspace.data_ptr(), workspace.data_ptr() + workspace.numel())
+    like = torch.empty(like.shape, dtype=like.dtype, device="cuda")
+    busy(side)
+    with torch.cuda.stream(side):
+        f(0, q, *args, out)
+    del f, workspace
+    assert not side.query() and not overlaps(span, like)
+    side.synchronize()
+    assert near(out, *reference(c, 0, q, range(4), 0.125))
+
+    d = pkg.PageCache(1, 30, 16, 2, 64, 4, 8)
+    spans = [(t, (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())) for t in (d.k, d.refs, d._work)]
+    spans = [(torch.empty_like(t), s) for t, s in spans]
+    torch.cuda.synchronize()
+    busy(side)
+    one, step = ints([1]), ints([0, 9])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        d.reserve(one, step)
+    del d
+    assert not side.query() and not any(overlaps(s, t) for t, s in spans)
+    side.synchronize()
