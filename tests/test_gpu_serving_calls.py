@@ -187,3 +187,40 @@ def test_memory_of_a_kernel_or_cache_dropped_while_another_stream_uses_it_is_not
     del d
     assert not side.query() and not any(overlaps(s, t) for t, s in spans)
     side.synchronize()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_a_query_that_is_not_finite_reaches_no_other_row_or_head(what, d):
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(300, h, d, generator=g).to(BF).cuda() for h in (4, 2, 2))
+    f, cu = pkg.kernels.make_prompt_attention_kernel(4, 2, d, 0.1), ints([0, 170, 300])
+    clean, out = torch.zeros_like(q), torch.zeros_like(q)
+    f(q, k, v, cu, clean)
+    q[100, 1, 3] = q[299, 2, 7] = what
+    f(q, k, v, cu, out)
+    for row, head in ((100, 1), (299, 2)):
+        assert out[row, head].isnan().all()
+        out[row, head] = clean[row, head]
+    # each within the bound of `near`, whose mass is at most the largest value
+    assert ((out.double() - clean.double()).abs() <= 2 * 1.02 * 2.0 ** -8 * (v.abs().max().item() + clean.double().abs())).all()
+    for heads, own in ((4, [[20, 0, 70], [5, 6]]), (96, [[20, 0, 70, 9], [5, 6]])):     # few and many columns
+        c, cu = branches([208, 100], own, 16, 2, d)
+        n = cu[-1]
+        a = pkg.make_prefix_attention_kernel(c, heads, 0.1, n, 2, 300)
+        q = torch.randn(n, heads, d, generator=g).to(BF).cuda()
+        out = torch.zeros_like(q)
+        ref, mass = reference(c, 0, q, range(n), 0.1)
+        q[1, 1, 3] = q[4, 2, 7] = what
+        a(0, q, ints(range(n)), ints(cu), ints([208, 100]), out)
+        for row, head in ((1, 1), (4, 2)):
+            assert out[row, head].isnan().all()
+            out[row, head], ref[row, head] = 0, 0
+        # not the same bits: the maximum of a wave's other queries moves when one of them has none
+        assert near(out, ref, mass)
+
+
+def test_rows_of_one_sequence_in_one_group_and_out_of_order():
+    """The same sequence in several rows, groups whose rows' sequences are in any order, and rows before and behind all groups."""
+    c, cu = branches([96, 48], [[20, 7, 0, 33], [5, 60]], 16, 2, 64)
+    check_attention(c, 8, [5, 3, 0, 3, 2, 1, 4, 5, 4, 0], [1, 6, 9], [96, 48])
