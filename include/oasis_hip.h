@@ -743,7 +743,7 @@ int oasis_video_decode(const oasis_dit_weights_t* w, const oasis_vae_weights_t* 
  * h / (n_heads / n_kv_heads). Keys, values, queries and outputs are bf16; scores, softmax
  * sums and partial results are fp32; the probabilities are rounded to bf16 for their product
  * with the values, and one below 2^-96 of the row's largest is taken as 0. Finite values give finite outputs: up to 2^127 in
- * magnitude over 2^22 keys, up to 2^120 over any number. scale is positive and finite.
+ * magnitude over 2^22 keys, up to 2^120 over any number. scale is positive and, times log2 e, finite.
  * Device-side integers are checked where they are used: nothing outside the buffers is read
  * or written, whatever they hold.
  * ==================================================================== */

@@ -892,7 +892,8 @@ extern "C" int oasis_pages_attention(const oasis_page_cache_t* cache, int64_t la
   OASIS_REQUIRE(sizes_ok(n_rows, n_groups, max_len, n_heads, hk, D), OASIS_ERR_SHAPE, "pages_attention: bad shape");
   OASIS_REQUIRE(layer >= 0 && layer < cache->n_layers, OASIS_ERR_SHAPE, "pages_attention: layer %lld of %lld",
                 (long long)layer, (long long)cache->n_layers);
-  OASIS_REQUIRE(scale > 0 && scale < INFINITY, OASIS_ERR_ARG, "pages_attention: the scale must be positive and finite");
+  OASIS_REQUIRE(scale > 0 && scale * flash::LOG2E < INFINITY, OASIS_ERR_ARG,
+                "pages_attention: the scale must be positive and finite");
   if (n_rows == 0) return OASIS_OK;
   OASIS_REQUIRE(q && out && seqs && (n_groups == 0 || (cu_groups && prefix_lens)), OASIS_ERR_NULL,
                 "pages_attention: null pointer");

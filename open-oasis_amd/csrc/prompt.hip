@@ -160,7 +160,8 @@ extern "C" int oasis_prompt_attention(const void* q, int64_t ld_q, const void* k
                 "prompt_attention: n_heads must be a multiple of n_kv_heads, up to 4096");
   OASIS_REQUIRE(n >= 0 && total >= 0 && n <= 65536 && total < (1ll << 30), OASIS_ERR_SHAPE,
                 "prompt_attention: bad sequence or token count");
-  OASIS_REQUIRE(scale > 0 && scale < INFINITY, OASIS_ERR_ARG, "prompt_attention: the scale must be positive and finite");
+  OASIS_REQUIRE(scale > 0 && scale * flash::LOG2E < INFINITY, OASIS_ERR_ARG,
+                "prompt_attention: the scale must be positive and finite");
   if (n == 0 || total == 0) return OASIS_OK;
   OASIS_REQUIRE(q && k && v && out && cu, OASIS_ERR_NULL, "prompt_attention: null pointer");
   OASIS_REQUIRE(ld_q >= n_heads * head_dim && ld_out >= n_heads * head_dim && ld_k >= n_kv_heads * head_dim &&

@@ -86,3 +86,12 @@ def test_calls_of_more_workgroups_than_a_launch_has_are_refused(name, args, need
     h = L.lib()
     rc = getattr(h, name)(*args)
     assert rc == SHAPE and needle in h.oasis_last_error().decode(), (rc, h.oasis_last_error())
+
+
+def test_a_scale_whose_product_with_log2_e_is_infinite_is_refused():
+    h = L.lib()
+    for scale, refused in ((3e38, True), (2.36e38, True), (float("inf"), True), (2.3e38, False)):
+        for name, args in (("oasis_prompt_attention", (None, 64, FAKE, 64, FAKE, 64, FAKE, 64, FAKE, 1, 1, 1, 1, 64, scale, None)),
+                           ("oasis_pages_attention", (cache(), 0, None, 128, FAKE, 128, FAKE, 1, None, None, 0, 10, 2, scale, None, 0, None))):
+            rc = getattr(h, name)(*args)
+            assert rc == (-5 if refused else -1) and ("scale" if refused else "null") in h.oasis_last_error().decode(), (name, scale)
